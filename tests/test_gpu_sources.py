@@ -1,0 +1,44 @@
+"""What no GPU code of this repository does, in the library, in the tools and in the kernel variants kept as text: it does not write
+through the scalar data cache (scalar stores and atomics, that cache's write-back and discard).  Vector stores do all writing.
+Measured results that mention such instructions stay in profiles/, which holds records and no code."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CODE = (".hip", ".h", ".hpp", ".c", ".cpp", ".py", ".sh", ".s", ".S", ".patch", ".diff", ".txt", ".mk", ".cfg", ".ini", ".cmake")
+TREES = ("nanocall_amd", "include", "oracle", "tools", "tests")
+SCALAR_WRITE = re.compile(r"\bs_(?:buffer_|scratch_)?(?:store|atomic)|\bs_dcache_(?:wb|discard)")
+
+
+def sources():
+    """(path, text) of every source, script and build file, found by walking (a copy of the tree without its history has them too)"""
+    top = [os.path.join(ROOT, f) for f in os.listdir(ROOT)]
+    paths = [p for p in top if os.path.isfile(p)]
+    for tree in TREES:
+        for d, dirs, files in os.walk(os.path.join(ROOT, tree)):
+            dirs[:] = [x for x in dirs if not x.startswith((".", "_")) and x != "build"]
+            paths += [os.path.join(d, f) for f in files]
+    for p in sorted(paths):
+        if p.endswith(CODE) or os.path.basename(p) == "Makefile":
+            with open(p, encoding="utf-8", errors="replace") as f:
+                yield os.path.relpath(p, ROOT), f.read()
+
+
+def lines(pattern):
+    return [f"{p}:{n}: {l.strip()[:120]}" for p, text in sources() for n, l in enumerate(text.split("\n"), 1) if pattern.search(l)]
+
+
+def test_the_walk_sees_the_code():
+    seen = {p for p, _ in sources()}
+    assert {"nanocall_amd/csrc/viterbi_kernel.hip", "nanocall_amd/csrc/Makefile", "bench.py", "tools/isa_budget.py", "tools/ubench/valu_rate.hip"} <= seen
+
+
+def test_the_pattern_knows_the_instructions():
+    for op in ("store_dword", "store_dwordx4", "buffer_store_dword", "scratch_store_dword", "atomic_add", "buffer_atomic_swap", "dcache_wb", "dcache_discard_x2"):
+        assert SCALAR_WRITE.search("s_" + op)
+    for op in ("s_load_dwordx4", "s_buffer_load_dword", "s_dcache_inv", "ds_store_b32", "global_store_dword", "buffer_store_dword", "global_atomic_add", "s_memtime"):
+        assert not SCALAR_WRITE.search("\t" + op)
+
+
+def test_no_source_writes_through_the_scalar_cache():
+    assert lines(SCALAR_WRITE) == []

@@ -33,7 +33,7 @@ def klass(op):
         return "lds"
     if op.startswith(("global_", "buffer_", "scratch_", "flat_")):
         return "vmem"
-    if op.startswith(("s_load", "s_store", "s_buffer", "s_dcache", "s_memtime", "s_memrealtime")):
+    if op.startswith(("s_load", "s_buffer_load", "s_memtime", "s_memrealtime")):
         return "smem"
     if op.startswith(("s_cbranch", "s_branch", "s_waitcnt", "s_nop", "s_barrier", "s_setprio", "s_endpgm", "s_sleep")):
         return "ctl"
