@@ -303,6 +303,10 @@ __device__ __forceinline__ void traceback_block(const ViterbiArgs& P, TbShared<T
             __syncthreads();
         }
         any_bad |= __syncthreads_or(on && q == 0 && T.bad[seg] != 0);
+        // (The width is stated: left to the vectorizer's own choice, which goes by the width of float arithmetic, it is 2, and the
+        // register allocation that follows costs the one-read column loop two more LDS waits per event: 5000 events on one CU
+        // 4.19 ms against 3.97 ms.)
+#pragma clang loop vectorize_width(4) interleave_count(1)
         for (int idx = (int)tid; idx < count; idx += THREADS) {
             const int w = idx / L;
             os[top - 1 - idx] = T.path[w][idx - w * L];

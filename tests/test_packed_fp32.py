@@ -75,3 +75,25 @@ def test_no_packed_fp32_in_the_built_library(tmp_path):
         if PACKED.search(text):
             found[f] = len(PACKED.findall(text))
     assert instructions > 1000 and not found, (instructions, found)
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not found")
+def test_kernels_without_packed_fp32_are_the_same_code_either_way(tmp_path):
+    """switching the feature off must not move anything else: where it changed a vectorizer's choice in the traceback, the one-read
+    column loop lost 5 % to other registers.  (The build with the feature is only compared as text.)"""
+    flags = _hipflags() + ["-S", "--cuda-device-only"]
+    i = next(i for i in range(len(flags)) if flags[i:i + 4] == OFF)
+    builds = {"off": flags, "on": flags[:i] + flags[i + 4:]}
+
+    def instructions(job):
+        name, which = job
+        out = tmp_path / f"{name}.{which}.s"
+        subprocess.run([HIPCC] + builds[which] + [name + ".hip", "-o", str(out)], cwd=CSRC, check=True, capture_output=True, timeout=900)
+        code = [l.split(";")[0].strip() for l in out.read_text().split("\n")]
+        return [l for l in code if l and not l.startswith((".", "__hip_cuid"))]      # (the latter: a label from the command line)
+
+    kernels = ("viterbi_kernel", "viterbi_ll_kernel", "emission_kernel", "fwbw_scaled_kernel", "em_kernel")
+    with ThreadPoolExecutor(4) as ex:
+        got = list(ex.map(instructions, [(k, w) for k in kernels for w in ("off", "on")]))
+    for n, k in enumerate(kernels):
+        assert got[2 * n] == got[2 * n + 1], k
