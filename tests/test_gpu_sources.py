@@ -42,3 +42,19 @@ def test_the_pattern_knows_the_instructions():
 
 def test_no_source_writes_through_the_scalar_cache():
     assert lines(SCALAR_WRITE) == []
+
+
+# ---- kernel variants kept as text ----
+def test_a_variant_keeps_every_barrier_and_bounds_check_of_its_kernel():
+    """tools/ubench/variants/*.hip.txt are compiled in place of the tree's kernel and run; the first line names that kernel"""
+    folder = os.path.join(ROOT, "tools", "ubench", "variants")
+    for f in sorted(os.listdir(folder)):
+        if f.endswith(".hip.txt"):
+            variant = open(os.path.join(folder, f)).read()
+            kernel = open(os.path.join(ROOT, "nanocall_amd", "csrc", re.match(r"// (\w+\.hip) ", variant).group(1))).read()
+            for guard in ("__syncthreads", "P.em_rows", "wave_barrier", "kNoSlot"):
+                assert variant.count(guard) >= kernel.count(guard), (f, guard, variant.count(guard), kernel.count(guard))
+
+
+def test_no_recipe_builds_a_kernel_without_its_barriers():
+    assert lines(re.compile(r"\bNCHMM_EXP_NO[A-Z]+\b")) == []
