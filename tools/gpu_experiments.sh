@@ -20,7 +20,7 @@ import sys, json
 d = json.loads(sys.stdin.read().strip().splitlines()[-1]); print('budget_mb=$mb', 'Mevents/s', d['value'], 'ms/step', d['ms_per_step'], 'launches', d['config']['forward_launches_per_step'])"
   done ;;
 rates)
-  (cd tools/ubench && hipcc --offload-arch=gfx950 -O3 valu_rate.hip -o valu_rate && ./valu_rate) | tee gpurun_out/valu_rate.txt ;;
+  (cd tools/ubench && hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate && ./valu_rate) | tee gpurun_out/valu_rate.txt ;;
 hbm)
   python tools/ubench/hbm_rate.py | tee gpurun_out/hbm_rate.txt ;;
 hostpath)

@@ -1,6 +1,6 @@
 // cu_stream_rate.hip -- how fast ONE CU takes in a stream of 16 KiB rows (the shape of "emissions ahead": 1024 threads, one
 // float4 per thread and row, rows consumed in order), by where the rows are and how many are in flight per thread.
-//   hipcc --offload-arch=gfx950 -O3 cu_stream_rate.hip -o cu_stream_rate && ./cu_stream_rate
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops cu_stream_rate.hip -o cu_stream_rate && ./cu_stream_rate
 // Columns: rows in flight (a burst of that many row loads per thread, all waited for, then the next burst), GB/s per CU and ns per row for
 //   L2      a 2 MiB ring read over and over (stays in the XCD's L2)
 //   MALL    a 128 MiB buffer read twice, second pass timed (fits the 256 MiB memory-side cache)

@@ -15,7 +15,7 @@
 // Output: div2_table.bin.nstar -- uint32 pairs (divisor significand, failing numerator significand), sorted; and
 //         div2_table.bin -- sorted uint32 entries (significand << 8) | code for the divisors whose plain pair does not work,
 // code 1..24 = the variant (variant_pair below) that does, 255 = none does (such a divisor keeps the 3-operation division).
-// Build: hipcc --offload-arch=gfx950 -O3 -ffp-contract=off div2_exhaustive.hip -o div2_exhaustive ; ./div2_exhaustive [out.bin]
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off div2_exhaustive.hip -o div2_exhaustive ; ./div2_exhaustive [out.bin]
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

@@ -7,7 +7,7 @@
 //   sleep1       one wave per CU looping on s_sleep            (the GPU is "busy", the VALUs are not)
 //   sleepfull    every wave slot looping on s_sleep
 //   valu1        one wave per SIMD running FMAs
-// hipcc --offload-arch=gfx950 -O3 -o keep_warm keep_warm.hip && ./keep_warm
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o keep_warm keep_warm.hip && ./keep_warm
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <cstdio>

@@ -1,6 +1,6 @@
 // valu_rate.hip -- VALU issue-rate microbenchmark for gfx950: cycles per wave-instruction of
-// v_fma_f32, v_pk_fma_f32, v_add_f32 + v_cndmask, at 1/2/4 waves per SIMD (one block per CU).
-// Build: hipcc --offload-arch=gfx950 -O3 valu_rate.hip -o valu_rate ; run on the GPU box.
+// v_fma_f32, v_add_f32, v_cndmask and others, at 1/2/4 waves per SIMD (one block per CU).
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
@@ -10,9 +10,7 @@ __global__ void k(float* out, int iters)
 {
     float a[8], b = 1.0001f, c = 0.5f;
     for (int i = 0; i < 8; ++i) a[i] = threadIdx.x * 0.001f + i;
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    f2 p[8]; for (int i = 0; i < 8; ++i) p[i] = f2{a[i], a[i] + 1};
-    f2 pb = {b, b}, pc = {c, c};
+    float p[8]; for (int i = 0; i < 8; ++i) p[i] = a[i];
     unsigned long long m2;
     unsigned long long msk = 0x5555555555555555ull ^ (unsigned long long)iters;
     if (MODE == 16) asm volatile("s_mov_b64 vcc, %0" :: "s"(msk) : "vcc");
@@ -24,12 +22,10 @@ __global__ void k(float* out, int iters)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (MODE == 0) asm volatile("v_fma_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
-                if (MODE == 1) asm volatile("v_pk_fma_f32 %0, %0, %1, %2" : "+v"(p[i]) : "v"(pb), "v"(pc));
                 if (MODE == 2) asm volatile("v_add_f32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 3) asm volatile("v_cndmask_b32 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : );
                 if (MODE == 4) asm volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
                 if (MODE == 5) asm volatile("v_cmp_gt_f32 vcc, %0, %1" : : "v"(a[i]), "v"(b) : "vcc");
-                if (MODE == 6) asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(p[i]) : "v"(pb));
                 if (MODE == 7) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 8) asm volatile("v_cndmask_b32_e64 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "s"(msk));
                 if (MODE == 9) asm volatile("v_cmp_gt_f32 vcc, %0, %1\n\tv_cndmask_b32 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : "vcc");
@@ -38,11 +34,11 @@ __global__ void k(float* out, int iters)
                 if (MODE == 12) asm volatile("v_lshl_or_b32 %0, %0, 1, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 13) asm volatile("v_rcp_f32 %0, %0" : "+v"(a[i]));
                 if (MODE == 14) asm volatile("v_cmp_gt_f32 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
-                if (MODE == 15) asm volatile("v_cmp_gt_f32 vcc, %0, %1\n\tv_cndmask_b32 %0, %0, %1, vcc\n\tv_cndmask_b32 %2, %2, %1, vcc" : "+v"(a[i]), "+v"(p[i].x) : "v"(b) : "vcc");
+                if (MODE == 15) asm volatile("v_cmp_gt_f32 vcc, %0, %1\n\tv_cndmask_b32 %0, %0, %1, vcc\n\tv_cndmask_b32 %2, %2, %1, vcc" : "+v"(a[i]), "+v"(p[i]) : "v"(b) : "vcc");
                 if (MODE == 17) asm volatile("v_cndmask_b32_e64 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : );
                 if (MODE == 18) asm volatile("v_cndmask_b32 %0, %1, %2, vcc" : "=v"(a[i]) : "v"(b), "v"(c) : );
                 if (MODE == 19) asm volatile("v_cmp_gt_f32 %1, %0, %2\n\tv_cndmask_b32_e64 %0, %0, %2, %1" : "+v"(a[i]), "=&s"(m2) : "v"(b));
-                if (MODE == 20) asm volatile("v_cmp_gt_f32 %2, %0, %3\n\tv_cndmask_b32_e64 %0, %0, %3, %2\n\tv_cndmask_b32_e64 %1, %1, %3, %2" : "+v"(a[i]), "+v"(p[i].x), "=&s"(m2) : "v"(b));
+                if (MODE == 20) asm volatile("v_cmp_gt_f32 %2, %0, %3\n\tv_cndmask_b32_e64 %0, %0, %3, %2\n\tv_cndmask_b32_e64 %1, %1, %3, %2" : "+v"(a[i]), "+v"(p[i]), "=&s"(m2) : "v"(b));
                 if (MODE == 16) asm volatile("v_cndmask_b32 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : );
                 if (MODE == 21) asm volatile("v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:1" : "+v"(a[i]));
                 if (MODE == 22) asm volatile("v_exp_f32 %0, %0" : "+v"(a[i]));
@@ -58,7 +54,7 @@ __global__ void k(float* out, int iters)
         }
     }
     long long t1 = clock64();
-    float s = 0; for (int i = 0; i < 8; ++i) s += a[i] + p[i].x + p[i].y;
+    float s = 0; for (int i = 0; i < 8; ++i) s += a[i] + p[i];
     out[blockIdx.x * blockDim.x + threadIdx.x] = s;
     if (threadIdx.x == 0 && blockIdx.x == 0) {
         ((long long*)out)[400000] = t1 - t0;                                   // shader cycles (s_memtime)
@@ -113,13 +109,10 @@ int main()
     sweep<26>("v_cmp_eq->sgpr", d);
     sweep<4>("v_max3_f32", d);
     sweep<22>("v_exp_f32", d);
-    sweep<1>("v_pk_fma_f32", d);
     for (int threads : {256, 512, 1024}) {
         run<0>("v_fma_f32", d, threads);
-        run<1>("v_pk_fma_f32", d, threads);
         run<2>("v_add_f32", d, threads);
         run<7>("v_mul_f32", d, threads);
-        run<6>("v_pk_mul_f32", d, threads);
         run<3>("v_cndmask_b32", d, threads);
         run<4>("v_max3_f32", d, threads);
         run<5>("v_cmp_gt_f32", d, threads);

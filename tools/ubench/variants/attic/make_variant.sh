@@ -1,9 +1,9 @@
 #!/bin/bash
 # Rebuild one of the measured-and-dropped kernel variants as it was measured: a worktree of the commit the variant was
-# derived from, the variant's patch applied to that commit's kernel, built there.  Run in the development container (it needs
-# the git history; the GPU box has none), then point gpurun at the worktree's library:
-#   tools/ubench/variants/make_variant.sh viterbi_split_barrier_kernel        -> /tmp/nc_variant_<name>/nanocall_amd/libnanocall_hip.so
-# The shipped tree is never patched (an interrupted in-place patch left a half-patched kernel behind).
+# derived from, the variant's patch applied to that commit's kernel, built there with the tree's own compiler
+# flags (no packed float32).  It needs the git history.
+#   tools/ubench/variants/attic/make_variant.sh viterbi_split_barrier_kernel        -> /tmp/nc_variant_<name>/nanocall_amd/libnanocall_hip.so
+# The shipped tree is never patched (an interrupted patch in place leaves a half-patched kernel behind).
 set -euo pipefail
 name=$1
 here=$(cd "$(dirname "$0")" && pwd)
@@ -16,5 +16,5 @@ wt=/tmp/nc_variant_$name
 rm -rf "$wt"; git -C "$root" worktree prune
 git -C "$root" worktree add -q --detach "$wt" "$commit"
 patch -s "$wt/$file" "$patch_file"
-make -s -C "$wt/nanocall_amd/csrc" -j8
+make -s -C "$wt/nanocall_amd/csrc" -j8 HIPFLAGS="$(make -s -C "$root/nanocall_amd/csrc" print-hipflags)"
 echo "$wt/nanocall_amd/libnanocall_hip.so  (commit $commit + $name.patch)"

@@ -7,8 +7,7 @@ REPS=${REPS:-3}
 cd $R/nanocall_amd/csrc
 # whatever ends this script (an error, an interrupt, a time limit): the tree's own object is rebuilt, never a variant's left behind
 trap 'rm -f viterbi_kernel.o; make -s > /dev/null 2>&1' EXIT
-FLAGS=$(make -s print-hipflags 2>/dev/null)
-[ -z "$FLAGS" ] && FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -I../../include -I. -Wall -Wno-unused-result -fno-slp-vectorize"
+FLAGS=$(make -s print-hipflags)
 line() { python -c "
 import sys, json
 d = json.loads(sys.stdin.read().strip().splitlines()[-1]); print('$1 Mevents/s', d['value'], 'ms_per_step', d['ms_per_step'], 'kernel_ms', d['roofline']['kernel_ms'], 'clock', d['device']['shader_clock_mhz_under_load'], 'cycles/step (M)', round(d['ms_per_step'] * d['device']['shader_clock_mhz_under_load'] / 1e3, 2))"; }

@@ -3,7 +3,7 @@
 #   FLAGSETS="-O3;-O3 -mllvm -amdgpu-enable-max-ilp-scheduling-strategy=1" bash tools/ubench/vit_flags.sh
 R=${GRAFT_REPO_ROOT:-$(pwd)}
 cd $R/nanocall_amd/csrc
-BASEF="--offload-arch=gfx950 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -I../../include -I. -Wall -Wno-unused-result -fno-slp-vectorize"
+BASEF=$(make -s print-hipflags | sed "s/ -O3 / /")
 IFS=';' read -ra SETS <<< "${FLAGSETS:--O3}"
 for f in "${SETS[@]}"; do
   echo "== $f"

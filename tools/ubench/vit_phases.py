@@ -19,7 +19,7 @@ import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 CSRC = os.path.join(ROOT, "nanocall_amd", "csrc")
-FLAGS = "--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -I../../include -I. -Wall -Wno-unused-result -fno-slp-vectorize".split()
+FLAGS = subprocess.run(["make", "-s", "-C", CSRC, "print-hipflags"], check=True, capture_output=True, text=True).stdout.split()
 
 
 def sub1(s, old, new):

@@ -2,7 +2,7 @@
 # bench.py (no CPU baseline, no FB leg) plus the bit-exactness tests.   VARIANTS="BASE NCHMM_BP_SDWA" bash tools/ubench/vit_variant.sh
 R=${GRAFT_REPO_ROOT:-$(pwd)}
 cd $R/nanocall_amd/csrc
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -I../../include -I. -Wall -Wno-unused-result -fno-slp-vectorize"
+FLAGS=$(make -s print-hipflags)
 for v in ${VARIANTS:-BASE}; do
   /opt/rocm/bin/hipcc $FLAGS -D$v -c viterbi_kernel.hip -o viterbi_kernel.o && make -s > /dev/null 2>&1
   echo "== $v"
