@@ -77,3 +77,10 @@ def test_every_build_of_gpu_code_switches_packed_fp32_off():
             assert p.startswith("tests/") or not BUILD_LINE.search(l) or "-Xclang -packed-fp32-ops" in l, f"{p}: {l.strip()}"
         if re.search(r"/hipcc\"?\]?\s*(?:\+\s*)?(?:\$FLAGS|\$BASEF|FLAGS|flags)\b", text):
             assert "print-hipflags" in text, p
+
+
+def test_the_variant_script_finds_the_repository():
+    """its patches are next to it, and the root that it works from is this tree"""
+    path = os.path.join(ROOT, "tools", "ubench", "variants", "attic", "make_variant.sh")
+    up = re.search(r'^root=\$\(cd "\$here/([./]+)"', open(path).read(), re.M).group(1)
+    assert os.path.realpath(os.path.join(os.path.dirname(path), up)) == os.path.realpath(ROOT)

@@ -7,7 +7,7 @@
 set -euo pipefail
 name=$1
 here=$(cd "$(dirname "$0")" && pwd)
-root=$(cd "$here/../../.." && pwd)
+root=$(cd "$here/../../../.." && pwd)
 patch_file=$here/$name.patch
 [ -f "$patch_file" ] || { echo "no such variant: $name" >&2; exit 2; }
 # "--- a/nanocall_amd/csrc/<file> (<commit>)"
