@@ -84,3 +84,50 @@ def test_the_variant_script_finds_the_repository():
     path = os.path.join(ROOT, "tools", "ubench", "variants", "attic", "make_variant.sh")
     up = re.search(r'^root=\$\(cd "\$here/([./]+)"', open(path).read(), re.M).group(1)
     assert os.path.realpath(os.path.join(os.path.dirname(path), up)) == os.path.realpath(ROOT)
+
+
+# ---- inline assembly: an operand that an instruction writes is declared as an output ----
+ASM = re.compile(r'\basm\b\s*(?:volatile\s*)?\(\s*((?:"(?:[^"\\]|\\.)*"\s*)+)(:.*)', re.S)
+
+
+def undeclared_writes(text):
+    """asm statements whose instructions write %N where N is an input (the compiler then believes that the input is unchanged)"""
+    found = []
+    for m in re.finditer(r"\basm\b\s*(?:volatile\s*)?\(", text):
+        a = ASM.match(text, m.start())
+        if not a:
+            continue
+        code = "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', a.group(1)))
+        outs, depth = "", 0
+        for ch in a.group(2)[1:]:
+            if ch == ":" and depth == 0 or ch == ")" and depth == 0:
+                break
+            depth += {"(": 1, "[": 1, ")": -1, "]": -1}.get(ch, 0)
+            outs += ch
+        n_out = len(re.findall(r'"[=+]', outs))
+        for ins in re.split(r"\\n\\t|\\n|;", code):
+            w = re.match(r"\s*(v_|s_|ds_read|ds_bpermute)(\S*)\s+(.*)", ins)
+            if not w or re.match(r"(nop|waitcnt|barrier|setprio|sleep|cmp)", w.group(2)) and w.group(1) == "s_":
+                continue
+            operands = [o.strip() for o in w.group(3).split(",")]
+            written = operands[:2] if "swap" in w.group(2) else operands[:1]
+            bad = [o for o in written if re.fullmatch(r"%\d+", o) and int(o[1:]) >= n_out]
+            if bad:
+                found.append((text.count("\n", 0, m.start()) + 1, ins.strip()))
+    return found
+
+
+def test_the_asm_check_sees_a_written_input():
+    assert undeclared_writes('asm volatile("v_add_f32 %0, %0, %1" : "+v"(a) : "v"(b));') == []
+    assert undeclared_writes('asm volatile("v_cmp_gt_f32_e64 %1, %0, %2" : : "v"(a[i]), "s"(m), "v"(b));') == [(1, "v_cmp_gt_f32_e64 %1, %0, %2")]
+    assert undeclared_writes('asm("v_max_f32 %0, %1, %2\\n\\tv_add_f32 %2, %1, %1" : "=v"(a) : "v"(f(b, c)), "v"(d));') == [(1, "v_add_f32 %2, %1, %1")]
+    assert undeclared_writes('asm("v_cmp_gt_f32 vcc, %0, %1\\n\\tv_cndmask_b32 %0, %0, %1, vcc" : "+v"(a) : "v"(b) : "vcc");') == []
+
+
+def test_inline_assembly_declares_what_it_writes():
+    seen = 0
+    for p, text in sources():
+        if p.endswith((".hip", ".hpp", ".h", ".hip.txt")) and not p.startswith("tests/"):
+            seen += len(re.findall(r"\basm\b", text))
+            assert undeclared_writes(text) == [], p
+    assert seen > 100

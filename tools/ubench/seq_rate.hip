@@ -40,18 +40,18 @@ __global__ __launch_bounds__(512, 4) void rate(float* out, int iters)
                 if (MODE == 14) asm volatile("v_writelane_b32 %0, %1, 5" : "+v"(a[i]) : "s"(sv));
                 if (MODE == 15) asm volatile("v_mov_b32 %0, %1" : "=v"(a[i]) : "s"(sv));
                 if (MODE == 16) asm volatile("v_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf" : "+v"(a[i]));
-                if (MODE == 17) asm volatile("v_cmp_eq_u32_e64 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
+                if (MODE == 17) asm volatile("v_cmp_eq_u32_e64 %0, %1, %2" : "+s"(msk) : "v"(a[i]), "v"(b));
                 if (MODE == 18) asm volatile("v_lshl_add_u32 %0, %0, 2, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 19) asm volatile("v_add3_u32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
                 if (MODE == 20) asm volatile("v_mad_u32_u24 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
                 if (MODE == 21) asm volatile("v_sub_f32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 22) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
-                if (MODE == 23) asm volatile("v_cmp_gt_f32_e64 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
+                if (MODE == 23) asm volatile("v_cmp_gt_f32_e64 %0, %1, %2" : "+s"(msk) : "v"(a[i]), "v"(b));
                 if (MODE == 24) asm volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
                 if (MODE == 25) asm volatile("v_lshl_or_b32 %0, %0, 8, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 26) asm volatile("v_mov_b32_dpp %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf" : "+v"(a[i]));
                 if (MODE == 27) asm volatile("v_and_b32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
-                if (MODE == 28) asm volatile("v_cmp_class_f32_e64 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
+                if (MODE == 28) asm volatile("v_cmp_class_f32_e64 %0, %1, %2" : "+s"(msk) : "v"(a[i]), "v"(b));
                 if (MODE == 29) asm volatile("v_min3_u32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "v"(c));
                 if (MODE == 30) asm volatile("v_add_u32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 31) asm volatile("v_readlane_b32 %0, %1, 3" : "=s"(sv) : "v"(a[i]));
@@ -59,15 +59,15 @@ __global__ __launch_bounds__(512, 4) void rate(float* out, int iters)
                 if (MODE == 32) asm volatile("v_cndmask_b32_e32 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : );
                 if (MODE == 33) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %1" : : "v"(a[i]), "v"(b) : "vcc");
                 if (MODE == 34) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %1\n\tv_cndmask_b32_e32 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : "vcc");
-                if (MODE == 35) asm volatile("v_cmp_gt_f32_e64 %2, %0, %1\n\tv_cndmask_b32_e64 %0, %0, %1, %2" : "+v"(a[i]) : "v"(b), "s"(msk));
+                if (MODE == 35) asm volatile("v_cmp_gt_f32_e64 %1, %0, %2\n\tv_cndmask_b32_e64 %0, %0, %2, %1" : "+v"(a[i]), "+s"(msk) : "v"(b));
                 if (MODE == 37) asm volatile("v_cndmask_b32_e64 %0, 1.0, 2.0, %1" : "=v"(a[i]) : "s"(msk));
                 if (MODE == 38) asm volatile("v_max_i32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 39) asm volatile("v_pk_max_f16 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 40) asm volatile("v_cndmask_b32_sdwa %0, %0, %1, vcc dst_sel:BYTE_1 dst_unused:UNUSED_PRESERVE src0_sel:DWORD src1_sel:DWORD" : "+v"(a[i]) : "v"(b));
                 // sequences as the Viterbi kernel has them (time per SEQUENCE): one compare feeding two selects (a scan step), and a
                 // 3-way combine cell (max3, three equality compares, tie logic on the scalar unit, two selects)
-                if (MODE == 43) asm volatile("v_cmp_gt_f32_e64 %3, %0, %2\n\tv_cndmask_b32_e64 %0, %0, %2, %3\n\tv_cndmask_b32_e64 %1, %1, %2, %3"
-                                             : "+v"(a[i]), "+v"(c) : "v"(b), "s"(msk));
+                if (MODE == 43) asm volatile("v_cmp_gt_f32_e64 %2, %0, %3\n\tv_cndmask_b32_e64 %0, %0, %3, %2\n\tv_cndmask_b32_e64 %1, %1, %3, %2"
+                                             : "+v"(a[i]), "+v"(c), "+s"(msk) : "v"(b));
                 if (MODE == 44) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %2\n\tv_cndmask_b32_e32 %0, %0, %2, vcc\n\tv_cndmask_b32_e32 %1, %1, %2, vcc"
                                              : "+v"(a[i]), "+v"(c) : "v"(b) : "vcc");
                 if (MODE == 45) asm volatile("v_max3_f32 %1, %0, %2, %3\n\t"
@@ -113,12 +113,12 @@ __global__ __launch_bounds__(512, 4) void rate(float* out, int iters)
                                              "v_cmp_eq_f32_e32 vcc, %0, %1\n\tv_cndmask_b32_e64 %5, %3, %2, s[20:21]\n\tv_add_f32 %6, %6, %8\n\tv_cndmask_b32_e32 %0, %5, %8, vcc\n\tv_add_f32 %7, %7, %8\n\t"
                                              "s_and_b64 s[26:27], vcc, s[20:21]\n\ts_or_b64 s[24:25], vcc, s[20:21]\n\ts_and_b64 s[24:25], s[24:25], s[22:23]\n\ts_or_b64 s[26:27], s[26:27], s[24:25]\n\ts_or_b64 %4, %4, s[26:27]"
                                              : "+v"(a[i]), "+v"(c), "+v"(b), "+v"(d2), "+s"(msk), "=&v"(t5), "+v"(f7), "+v"(f8) : "v"(z6) : "vcc", "scc", "s20", "s21", "s22", "s23", "s24", "s25", "s26", "s27");
-                if (MODE == 57) asm volatile("v_cmp_gt_f32_e64 %3, %0, %2\n\tv_cndmask_b32_e64 %0, %0, %2, %3\n\tv_add_f32 %4, %4, %2\n\tv_cndmask_b32_e64 %1, %1, %2, %3"
-                                             : "+v"(a[i]), "+v"(c) : "v"(b), "s"(msk), "v"(f7));
+                if (MODE == 57) asm volatile("v_cmp_gt_f32_e64 %2, %0, %4\n\tv_cndmask_b32_e64 %0, %0, %4, %2\n\tv_add_f32 %3, %3, %4\n\tv_cndmask_b32_e64 %1, %1, %4, %2"
+                                             : "+v"(a[i]), "+v"(c), "+s"(msk), "+v"(f7) : "v"(b));
                 if (MODE == 58) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %2\n\tv_cndmask_b32_e32 %0, %0, %2, vcc\n\tv_nop\n\tv_cndmask_b32_e32 %1, %1, %2, vcc"
                                              : "+v"(a[i]), "+v"(c) : "v"(b) : "vcc");
-                if (MODE == 59) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %2\n\tv_cndmask_b32_e32 %0, %0, %2, vcc\n\tv_fma_f32 %3, %3, %2, %2\n\tv_cndmask_b32_e32 %1, %1, %2, vcc"
-                                             : "+v"(a[i]), "+v"(c) : "v"(b), "v"(f7) : "vcc");
+                if (MODE == 59) asm volatile("v_cmp_gt_f32_e32 vcc, %0, %3\n\tv_cndmask_b32_e32 %0, %0, %3, vcc\n\tv_fma_f32 %2, %2, %3, %3\n\tv_cndmask_b32_e32 %1, %1, %3, vcc"
+                                             : "+v"(a[i]), "+v"(c), "+v"(f7) : "v"(b) : "vcc");
                 // half-rate and full-rate ops interleaved, every chain independent (a[i] for the half-rate op, g[i] / h[i] / k[i] for the adds)
                 if (MODE == 60) asm volatile("v_max_f32 %0, %0, %2\n\tv_add_f32 %1, %1, %2" : "+v"(a[i]), "+v"(g[i]) : "v"(b));
                 if (MODE == 61) asm volatile("v_max_f32 %0, %0, %3\n\tv_add_f32 %1, %1, %3\n\tv_add_f32 %2, %2, %3" : "+v"(a[i]), "+v"(g[i]), "+v"(h[i]) : "v"(b));
@@ -141,16 +141,16 @@ __global__ __launch_bounds__(512, 4) void rate(float* out, int iters)
                 if (MODE == 76) asm volatile("v_cndmask_b32_e64 %0, %0, %2, %3\n\tv_fma_f32 %1, %1, %2, %2" : "+v"(a[i]), "+v"(g[i]) : "v"(b), "s"(msk));
                 if (MODE == 77) asm volatile("v_add_f32 %1, %1, %2\n\tv_cmp_gt_f32_e64 s[20:21], %0, %2" : "+v"(a[i]), "+v"(g[i]) : "v"(b) : "s20", "s21");
                 if (MODE == 78) asm volatile("v_cmp_eq_f32_e64 s[20:21], %0, %2\n\tv_cmp_eq_f32_e64 s[22:23], %1, %2" : "+v"(a[i]), "+v"(g[i]) : "v"(b) : "s20", "s21", "s22", "s23");
-                if (MODE == 79) asm volatile("v_cndmask_b32_e64 %0, %0, %3, %4\n\tv_sub_f32 %1, %1, %3\n\tv_cndmask_b32_e64 %2, %2, %3, %4\n\tv_mul_f32 %5, %5, %3"
-                                             : "+v"(a[i]), "+v"(g[i]), "+v"(h[i]) : "v"(b), "s"(msk), "v"(k[i]));
+                if (MODE == 79) asm volatile("v_cndmask_b32_e64 %0, %0, %4, %5\n\tv_sub_f32 %1, %1, %4\n\tv_cndmask_b32_e64 %2, %2, %4, %5\n\tv_mul_f32 %3, %3, %4"
+                                             : "+v"(a[i]), "+v"(g[i]), "+v"(h[i]), "+v"(k[i]) : "v"(b), "s"(msk));
                 // the combine cell with SIX independent full-rate riders (sub / mul / add), one after each half-rate op
-                if (MODE == 80) asm volatile("v_max3_f32 %1, %0, %2, %3\n\tv_sub_f32 %6, %6, %8\n\t"
-                                             "v_cmp_eq_f32_e64 s[20:21], %2, %1\n\tv_mul_f32 %7, %7, %8\n\t"
-                                             "v_cmp_eq_f32_e64 s[22:23], %3, %1\n\tv_sub_f32 %9, %9, %8\n\t"
-                                             "v_cmp_eq_f32_e64 s[28:29], %0, %1\n\tv_mul_f32 %10, %10, %8\n\t"
-                                             "v_cndmask_b32_e64 %5, %3, %2, s[20:21]\n\tv_add_f32 %6, %6, %8\n\tv_cndmask_b32_e64 %0, %5, 0, s[28:29]\n\tv_add_f32 %7, %7, %8\n\t"
+                if (MODE == 80) asm volatile("v_max3_f32 %1, %0, %2, %3\n\tv_sub_f32 %6, %6, %10\n\t"
+                                             "v_cmp_eq_f32_e64 s[20:21], %2, %1\n\tv_mul_f32 %7, %7, %10\n\t"
+                                             "v_cmp_eq_f32_e64 s[22:23], %3, %1\n\tv_sub_f32 %8, %8, %10\n\t"
+                                             "v_cmp_eq_f32_e64 s[28:29], %0, %1\n\tv_mul_f32 %9, %9, %10\n\t"
+                                             "v_cndmask_b32_e64 %5, %3, %2, s[20:21]\n\tv_add_f32 %6, %6, %10\n\tv_cndmask_b32_e64 %0, %5, 0, s[28:29]\n\tv_add_f32 %7, %7, %10\n\t"
                                              "s_and_b64 s[26:27], s[28:29], s[20:21]\n\ts_or_b64 s[24:25], s[28:29], s[20:21]\n\ts_and_b64 s[24:25], s[24:25], s[22:23]\n\ts_or_b64 s[26:27], s[26:27], s[24:25]\n\ts_or_b64 %4, %4, s[26:27]"
-                                             : "+v"(a[i]), "+v"(c), "+v"(b), "+v"(d2), "+s"(msk), "=&v"(t5), "+v"(g[i]), "+v"(h[i]) : "v"(z6), "v"(k[i]), "v"(f7)
+                                             : "+v"(a[i]), "+v"(c), "+v"(b), "+v"(d2), "+s"(msk), "=&v"(t5), "+v"(g[i]), "+v"(h[i]), "+v"(k[i]), "+v"(f7) : "v"(z6)
                                              : "vcc", "scc", "s20", "s21", "s22", "s23", "s24", "s25", "s26", "s27", "s28", "s29");
                 // transcendental + riders
                 if (MODE == 90) asm volatile("v_exp_f32 %0, %0" : "+v"(a[i]));

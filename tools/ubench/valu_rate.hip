@@ -33,8 +33,8 @@ __global__ void k(float* out, int iters)
                 if (MODE == 11) asm volatile("v_mov_b32 %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 12) asm volatile("v_lshl_or_b32 %0, %0, 1, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 13) asm volatile("v_rcp_f32 %0, %0" : "+v"(a[i]));
-                if (MODE == 14) asm volatile("v_cmp_gt_f32 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
-                if (MODE == 15) asm volatile("v_cmp_gt_f32 vcc, %0, %1\n\tv_cndmask_b32 %0, %0, %1, vcc\n\tv_cndmask_b32 %2, %2, %1, vcc" : "+v"(a[i]), "+v"(p[i]) : "v"(b) : "vcc");
+                if (MODE == 14) asm volatile("v_cmp_gt_f32 %0, %1, %2" : "+s"(msk) : "v"(a[i]), "v"(b));
+                if (MODE == 15) asm volatile("v_cmp_gt_f32 vcc, %0, %2\n\tv_cndmask_b32 %0, %0, %2, vcc\n\tv_cndmask_b32 %1, %1, %2, vcc" : "+v"(a[i]), "+v"(p[i]) : "v"(b) : "vcc");
                 if (MODE == 17) asm volatile("v_cndmask_b32_e64 %0, %0, %1, vcc" : "+v"(a[i]) : "v"(b) : );
                 if (MODE == 18) asm volatile("v_cndmask_b32 %0, %1, %2, vcc" : "=v"(a[i]) : "v"(b), "v"(c) : );
                 if (MODE == 19) asm volatile("v_cmp_gt_f32 %1, %0, %2\n\tv_cndmask_b32_e64 %0, %0, %2, %1" : "+v"(a[i]), "=&s"(m2) : "v"(b));
@@ -45,7 +45,7 @@ __global__ void k(float* out, int iters)
                 if (MODE == 23) asm volatile("v_and_b32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 24) asm volatile("v_bfe_i32 %0, %0, 3, 1" : "+v"(a[i]));
                 if (MODE == 25) asm volatile("v_min_f32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
-                if (MODE == 26) asm volatile("v_cmp_eq_f32 %1, %0, %2" : : "v"(a[i]), "s"(msk), "v"(b));
+                if (MODE == 26) asm volatile("v_cmp_eq_f32 %0, %1, %2" : "+s"(msk) : "v"(a[i]), "v"(b));
                 if (MODE == 27) asm volatile("v_add_u32 %0, %0, %1" : "+v"(a[i]) : "v"(b));
                 if (MODE == 28) asm volatile("v_fma_f32 %0, %0, %2, %3\n\tv_cmp_gt_f32 %1, %0, %2" : "+v"(a[i]), "=&s"(m2) : "v"(b), "v"(c));
                 if (MODE == 29) asm volatile("v_mov_b32_dpp %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf" : "+v"(a[i]));
